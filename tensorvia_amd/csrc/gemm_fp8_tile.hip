@@ -439,13 +439,15 @@ void gemm_fp8_tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n, int group_m, Fp8S
     }
 }
 
-// The loaders add 32-bit offsets to a tile's base (for gathered rows the operand's), which stay below 2^31 - 2^20.
+// The loaders add 32-bit offsets to a tile's base (for gathered rows the operand's), which stay below 2^31 - 2^20.  Among them are those
+// of the two k-tiles that the loop asks for past the end: their lanes are out of range, but the range check subtracts the
+// k-tile's scalar advance from the descriptor's size, so an advance beyond the size would let them through.
 bool fp8_tile_ok(const Fp8Gemm& g, int mode) {
     const int64_t lim = ((int64_t)1 << 31) - ((int64_t)1 << 20);
     const int64_t a_rows = mode == FP8_GATE_UP ? g.tokens : 256;
     const int64_t w_off = (mode == FP8_GATE_UP ? g.sw_g : 0) + 256 * g.sw_n + g.K;
     return fast_rows(g.A, g.M, g.sa_m, g.K) && fast_rows(g.W, g.N, g.sw_n, g.K) && g.sw_e % 16 == 0 && g.sw_g % 16 == 0 &&
-           a_rows * g.sa_m + g.K < lim && a_rows * g.sas_m * 4 + (g.K / 128 + 1) * g.sas_k * 4 < lim && w_off < lim && g.K > 0;
+           a_rows * g.sa_m + g.K < lim && a_rows * g.sas_m * 4 + (g.K / 128 + 2) * g.sas_k * 4 < lim && w_off < lim && g.K > 0;
 }
 
 // The operands as pad_fp8_operands leaves them, but for their addresses.
