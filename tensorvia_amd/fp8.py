@@ -7,7 +7,7 @@ consecutive elements of a row (activations: ``scale[m, k // 128]``) or of 128 x 
 [blocks, rows] tensor, transposed): that is how the products read them fastest.  Any strides are accepted.
 
 Like ``gemm``, every function is asynchronous on ``stream`` (default torch's current one), takes the
-tensors to write as optional arguments, and raises RuntimeError for arguments that do not fit together.
+tensors to write as optional arguments, and raises RuntimeError for arguments that do not fit together or are not on a GPU.
 """
 from __future__ import annotations
 
@@ -15,7 +15,7 @@ import struct
 
 import torch
 
-from . import BFLOAT16, FLOAT16, FLOAT32, FP8_BLOCK, check
+from . import BFLOAT16, FLOAT16, FLOAT32, FP8_BLOCK, TV_E_SHAPE, check
 from .matmul import _current_stream, _entry, _stream
 
 _F8 = torch.float8_e4m3fn
@@ -94,7 +94,9 @@ def _codes_out(q, shape: tuple, device) -> tuple:
     return q, _row(q, "q", _F8, shape, device)
 
 
-def _call(name: str, args: bytes, stream) -> None:
+def _call(name: str, args: bytes, device, stream) -> None:
+    if device.type != "cuda":
+        _fail(f"the tensors must be on a GPU, got {device}")
     rc = _entry(name)(args, _current_stream() if stream is None else _stream(stream))
     if rc:
         check(rc)
@@ -121,7 +123,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1, q: torch.Tensor | None = 
         _fail(f"block_rows must be 1 or {FP8_BLOCK}, got {block_rows}")
     q, sq = _codes_out(q, shape, dev)
     _call("tv_hip_quantize_fp8", _pack_quantize(dt, block_rows, m, k, x.data_ptr(), k if x.is_contiguous() else _rows(x, "x"),
-                                                q.data_ptr(), sq, scale.data_ptr(), *ss), stream)
+                                                q.data_ptr(), sq, scale.data_ptr(), *ss), dev, stream)
     return q, scale
 
 
@@ -163,7 +165,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     scale, ss = _scale_out(scale, (t, (h + 127) // 128), dev)
     _call("tv_hip_rms_norm_fp8",
           _pack_norm(dt, _FLOATS[dw], t, h, eps, 0, x.data_ptr(), h if x.is_contiguous() else _rows(x, "x"), pr, sr,
-                     weight.data_ptr(), q.data_ptr(), sq, scale.data_ptr(), *ss, po, so, pn, sn), stream)
+                     weight.data_ptr(), q.data_ptr(), sq, scale.data_ptr(), *ss, po, so, pn, sn), dev, stream)
     return q, scale, residual_out, normed
 
 
@@ -185,7 +187,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
     ws = _any(w_scale, "w_scale", torch.float32, ((n + 127) // 128, kb), dev)
     out, dt, so = _out(out, out_dtype, (m, n), dev)
     _call("tv_hip_gemm_fp8", _pack_gemm(dt, 0, m, n, k, a.data_ptr(), ra, a_scale.data_ptr(), *ss, w.data_ptr(), rw,
-                                        w_scale.data_ptr(), *ws, out.data_ptr(), so), stream)
+                                        w_scale.data_ptr(), *ws, out.data_ptr(), so), dev, stream)
     return out
 
 
@@ -207,6 +209,8 @@ def route(logits: torch.Tensor, k: int, scoring: str = "softmax", bias: torch.Te
     dt, (t, e), dev = _float(logits, "logits"), logits.shape, logits.device
     if scoring not in _SCORING:
         _fail(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    if not 1 <= k <= e:
+        check(TV_E_SHAPE)
     pb = 0 if bias is None else _dense(bias, "bias", torch.float32, (e,), dev)
     if weights is None:
         weights = torch.empty(t, k, dtype=torch.float32, device=dev)
@@ -215,7 +219,7 @@ def route(logits: torch.Tensor, k: int, scoring: str = "softmax", bias: torch.Te
     pw, pi = _dense(weights, "weights", torch.float32, (t, k), dev), _dense(ids, "ids", torch.int32, (t, k), dev)
     _call("tv_hip_route",
           _pack_route(dt, _SCORING[scoring], t, e, k, groups, topk_groups, group_top, bool(renormalize), scale, 0,
-                      logits.data_ptr(), e if logits.is_contiguous() else _rows(logits, "logits"), pb, pw, pi), stream)
+                      logits.data_ptr(), e if logits.is_contiguous() else _rows(logits, "logits"), pb, pw, pi), dev, stream)
     return weights, ids
 
 
@@ -246,5 +250,5 @@ def experts_fp8(a: torch.Tensor, a_scale: torch.Tensor, w1: torch.Tensor, w1_sca
     out, dt, so = _out(out, out_dtype, (t, h), dev)
     _call("tv_hip_experts_fp8",
           _pack_experts(dt, 0, t, h, i, e, k, a.data_ptr(), ra, a_scale.data_ptr(), *ss, w1.data_ptr(), *t1[:3], p1,
-                        w2.data_ptr(), *t2[:2], p2, pw, pi, out.data_ptr(), so), stream)
+                        w2.data_ptr(), *t2[:2], p2, pw, pi, out.data_ptr(), so), dev, stream)
     return out
