@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import BFLOAT16, FLOAT16, FLOAT32, FP8_BLOCK, TV_E_SHAPE, check
-from .matmul import _current_stream, _entry, _stream
+from .matmul import _launch
 
 _F8 = torch.float8_e4m3fn
 _FLOATS = {torch.bfloat16: BFLOAT16, torch.float16: FLOAT16, torch.float32: FLOAT32}
@@ -97,7 +97,7 @@ def _codes_out(q, shape: tuple, device) -> tuple:
 def _call(name: str, args: bytes, device, stream) -> None:
     if device.type != "cuda":
         _fail(f"the tensors must be on a GPU, got {device}")
-    rc = _entry(name)(args, _current_stream() if stream is None else _stream(stream))
+    rc = _launch(name, args, device, stream)
     if rc:
         check(rc)
 

@@ -138,12 +138,23 @@ def _stream_getter():
 
 
 _current_stream = _stream_getter()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(stream) -> int:
     if stream is None:
         return _current_stream()
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _launch(name: str, args: bytes, device: torch.device, stream) -> int:
+    """The entry point's code.  The library launches on the current device, with that one's workspace, so a call on another
+    device's tensors makes it the current one."""
+    index = device.index
+    if index is not None and index != _current_device():  # None: host tensors
+        with torch.cuda.device(index):
+            return _entry(name)(args, _current_stream() if stream is None else _stream(stream))
+    return _entry(name)(args, _current_stream() if stream is None else _stream(stream))
 
 
 def _run(name: str, a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None, out_dtype: int | None, stream) -> torch.Tensor:
@@ -168,7 +179,7 @@ def _run(name: str, a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None, 
     else:
         args = _pack_args(da, db, dc, 0, 1, m, n, k, a.data_ptr(), 0, *a.stride(), b.data_ptr(), 0, *b.stride(),
                           out.data_ptr(), 0, *out.stride())
-    check(_entry(name)(args, _current_stream() if stream is None else _stream(stream)))
+    check(_launch(name, args, a.device, stream))
     return out
 
 
@@ -187,5 +198,5 @@ def gemv(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None, out_
 def matmul(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """``ops::Mul`` / ``ops::matmul``: synchronous, like the reference (src/backend/cuda/mul.cu:122)."""
     c = gemm(a, b)
-    torch.cuda.current_stream().synchronize()
+    torch.cuda.current_stream(c.device).synchronize()
     return c
