@@ -6,8 +6,8 @@ consecutive elements of a row (activations: ``scale[m, k // 128]``) or of 128 x 
 ``scale[n // 128, k // 128]``).  The activation scales that these functions allocate are stored by column (a
 [blocks, rows] tensor, transposed): that is how the products read them fastest.  Any strides are accepted.
 
-Like ``gemm``, every function is asynchronous on ``stream`` (default torch's current one), takes the
-tensors to write as optional arguments, and raises RuntimeError for arguments that do not fit together or are not on a GPU.
+Like ``gemm``, every function is asynchronous on ``stream`` (default torch's current one; what it allocates then
+belongs to that stream), takes the tensors to write as optional arguments, and raises RuntimeError for arguments that do not fit together or are not on a GPU.
 """
 from __future__ import annotations
 
@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import BFLOAT16, FLOAT16, FLOAT32, FP8_BLOCK, TV_E_SHAPE, check
-from .matmul import _launch
+from .matmul import _empty, _launch
 
 _F8 = torch.float8_e4m3fn
 _FLOATS = {torch.bfloat16: BFLOAT16, torch.float16: FLOAT16, torch.float32: FLOAT32}
@@ -70,27 +70,27 @@ def _dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device)
     return t.data_ptr()
 
 
-def _out(out, out_dtype, shape: tuple, device) -> tuple:
+def _out(out, out_dtype, shape: tuple, device, stream) -> tuple:
     """The result tensor, its type and its row stride."""
     if out is None:
         out_dtype = BFLOAT16 if out_dtype is None else out_dtype
         if out_dtype not in _TORCH:
             _fail(f"out_dtype must be BFLOAT16, FLOAT16 or FLOAT32, got {out_dtype}")
-        return torch.empty(shape, dtype=_TORCH[out_dtype], device=device), out_dtype, shape[1]
+        return _empty(shape, _TORCH[out_dtype], device, stream), out_dtype, shape[1]
     dt = _float(out, "out")
     return out, dt, _row(out, "out", out.dtype if out_dtype is None else _TORCH.get(out_dtype), shape, device)
 
 
-def _scale_out(scale, shape: tuple, device) -> tuple:
+def _scale_out(scale, shape: tuple, device, stream) -> tuple:
     """Activation scales, stored by column where they are made here, and their strides."""
     if scale is None:
-        return torch.empty(shape[1], shape[0], dtype=torch.float32, device=device).t(), (1, shape[0])
+        return _empty((shape[1], shape[0]), torch.float32, device, stream).t(), (1, shape[0])
     return scale, _any(scale, "scale", torch.float32, shape, device)
 
 
-def _codes_out(q, shape: tuple, device) -> tuple:
+def _codes_out(q, shape: tuple, device, stream) -> tuple:
     if q is None:
-        return torch.empty(shape, dtype=_F8, device=device), shape[1]
+        return _empty(shape, _F8, device, stream), shape[1]
     return q, _row(q, "q", _F8, shape, device)
 
 
@@ -113,15 +113,15 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1, q: torch.Tensor | None = 
     dt, shape, dev = _float(x, "x"), x.shape, x.device
     m, k = shape
     if block_rows == 1:
-        scale, ss = _scale_out(scale, (m, (k + 127) // 128), dev)
+        scale, ss = _scale_out(scale, (m, (k + 127) // 128), dev, stream)
     elif block_rows == FP8_BLOCK:
         grid = ((m + 127) // 128, (k + 127) // 128)
         if scale is None:
-            scale = torch.empty(grid, dtype=torch.float32, device=dev)
+            scale = _empty(grid, torch.float32, dev, stream)
         ss = _any(scale, "scale", torch.float32, grid, dev)
     else:
         _fail(f"block_rows must be 1 or {FP8_BLOCK}, got {block_rows}")
-    q, sq = _codes_out(q, shape, dev)
+    q, sq = _codes_out(q, shape, dev, stream)
     _call("tv_hip_quantize_fp8", _pack_quantize(dt, block_rows, m, k, x.data_ptr(), k if x.is_contiguous() else _rows(x, "x"),
                                                 q.data_ptr(), sq, scale.data_ptr(), *ss), dev, stream)
     return q, scale
@@ -152,17 +152,17 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     if residual is not None:
         pr, sr = residual.data_ptr(), _row(residual, "residual", dtype, shape, dev)
         if residual_out is None:
-            residual_out = torch.empty(shape, dtype=dtype, device=dev)
+            residual_out = _empty(shape, dtype, dev, stream)
     if residual_out is not None:
         po, so = residual_out.data_ptr(), _row(residual_out, "residual_out", dtype, shape, dev)
     if normed is True:
-        normed = torch.empty(shape, dtype=dtype, device=dev)
+        normed = _empty(shape, dtype, dev, stream)
     elif normed is False:
         normed = None
     if normed is not None:
         pn, sn = normed.data_ptr(), _row(normed, "normed", dtype, shape, dev)
-    q, sq = _codes_out(q, shape, dev)
-    scale, ss = _scale_out(scale, (t, (h + 127) // 128), dev)
+    q, sq = _codes_out(q, shape, dev, stream)
+    scale, ss = _scale_out(scale, (t, (h + 127) // 128), dev, stream)
     _call("tv_hip_rms_norm_fp8",
           _pack_norm(dt, _FLOATS[dw], t, h, eps, 0, x.data_ptr(), h if x.is_contiguous() else _rows(x, "x"), pr, sr,
                      weight.data_ptr(), q.data_ptr(), sq, scale.data_ptr(), *ss, po, so, pn, sn), dev, stream)
@@ -185,7 +185,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
     kb = (k + 127) // 128
     ss = _any(a_scale, "a_scale", torch.float32, (m, kb), dev)
     ws = _any(w_scale, "w_scale", torch.float32, ((n + 127) // 128, kb), dev)
-    out, dt, so = _out(out, out_dtype, (m, n), dev)
+    out, dt, so = _out(out, out_dtype, (m, n), dev, stream)
     _call("tv_hip_gemm_fp8", _pack_gemm(dt, 0, m, n, k, a.data_ptr(), ra, a_scale.data_ptr(), *ss, w.data_ptr(), rw,
                                         w_scale.data_ptr(), *ws, out.data_ptr(), so), dev, stream)
     return out
@@ -213,9 +213,9 @@ def route(logits: torch.Tensor, k: int, scoring: str = "softmax", bias: torch.Te
         check(TV_E_SHAPE)
     pb = 0 if bias is None else _dense(bias, "bias", torch.float32, (e,), dev)
     if weights is None:
-        weights = torch.empty(t, k, dtype=torch.float32, device=dev)
+        weights = _empty((t, k), torch.float32, dev, stream)
     if ids is None:
-        ids = torch.empty(t, k, dtype=torch.int32, device=dev)
+        ids = _empty((t, k), torch.int32, dev, stream)
     pw, pi = _dense(weights, "weights", torch.float32, (t, k), dev), _dense(ids, "ids", torch.int32, (t, k), dev)
     _call("tv_hip_route",
           _pack_route(dt, _SCORING[scoring], t, e, k, groups, topk_groups, group_top, bool(renormalize), scale, 0,
@@ -247,7 +247,7 @@ def experts_fp8(a: torch.Tensor, a_scale: torch.Tensor, w1: torch.Tensor, w1_sca
     p1 = _dense(w1_scale, "w1_scale", torch.float32, (e, 2, ib, hb), dev)
     p2 = _dense(w2_scale, "w2_scale", torch.float32, (e, hb, ib), dev)
     pw, pi = _dense(weights, "weights", torch.float32, (t, k), dev), _dense(ids, "ids", torch.int32, (t, k), dev)
-    out, dt, so = _out(out, out_dtype, (t, h), dev)
+    out, dt, so = _out(out, out_dtype, (t, h), dev, stream)
     _call("tv_hip_experts_fp8",
           _pack_experts(dt, 0, t, h, i, e, k, a.data_ptr(), ra, a_scale.data_ptr(), *ss, w1.data_ptr(), *t1[:3], p1,
                         w2.data_ptr(), *t2[:2], p2, pw, pi, out.data_ptr(), so), dev, stream)

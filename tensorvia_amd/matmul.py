@@ -147,6 +147,18 @@ def _stream(stream) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """A result tensor that the call allocates, from the memory of the stream that writes it: memory that another stream freed may
+    still be in use by work queued there.  The caller's current stream may use the result too (once ordered behind `stream`),
+    so the memory is not handed out again before what that stream has queued by the time the tensor is freed."""
+    if stream is None or device.type != "cuda" or _stream(stream) == torch.cuda.current_stream(device).cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream):
+        out = torch.empty(shape, dtype=dtype, device=device)
+    out.record_stream(torch.cuda.current_stream(device))
+    return out
+
+
 def _launch(name: str, args: bytes, device: torch.device, stream) -> int:
     """The entry point's code.  The library launches on the current device, with that one's workspace, so a call on another
     device's tensors makes it the current one."""
@@ -170,7 +182,7 @@ def _run(name: str, a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None, 
     m, k, n = sa[-2], sa[-1], sb[-1]
     shape = (sa[0], m, n) if batched else (m, n)
     if out is None:
-        out = a.new_empty(shape, dtype=_TV2T[dc])
+        out = a.new_empty(shape, dtype=_TV2T[dc]) if stream is None else _empty(shape, _TV2T[dc], a.device, stream)
     elif tuple(out.shape) != shape or torch_to_tv(out.dtype) != dc:
         raise RuntimeError(f"out has shape {tuple(out.shape)}/{out.dtype}, expected {shape}/{tv_to_torch(dc)}")
     if batched:
@@ -185,7 +197,8 @@ def _run(name: str, a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None, 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None, out_dtype: int | None = None,
          stream=None) -> torch.Tensor:
-    """C = A @ B on the HIP kernels (asynchronous on ``stream``, default torch's current stream)."""
+    """C = A @ B on the HIP kernels (asynchronous on ``stream``, default torch's current stream; without ``out`` the result's
+    memory belongs to that stream, and the caller orders its use behind it)."""
     return _run("tv_hip_gemm", a, b, out, out_dtype, stream)
 
 
