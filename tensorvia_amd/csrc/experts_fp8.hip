@@ -233,8 +233,15 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
     // whose own rounding is 1.7e-3, go without (2.0e-3 together), and fp16 ones (3.3e-4) do not.
     up.exact = a.dtype_c != TV_BFLOAT16;
     bool tiled = tk >= (int64_t)(pad_up ? kPadTileRows : pad_down ? kPadDownTileRows : up.exact ? kExactTileRows : kTileRows) * a.E && a.dtype_c != TV_FLOAT32 && a.I > 0;
-    tiled = tiled && (!pad_down || fp8_pad_ok(down, FP8_DOWN));
-    if (tiled && pad_up) tiled = pad_fp8_operands(up, FP8_GATE_UP, stream) == 0;
+    tiled = tiled && (!pad_up || fp8_pad_ok(up, FP8_GATE_UP)) && (!pad_down || fp8_pad_ok(down, FP8_DOWN));
+    // One buffer holds W1's copy, then W2's.  Without room for it the other kernels run.
+    Fp8Pads pads{};
+    if (tiled && (pad_up || pad_down)) {
+        Fp8PadBytes bytes = pad_up ? fp8_pad_bytes(up, FP8_GATE_UP) : Fp8PadBytes{};
+        const size_t w2 = pad_down ? fp8_pad_bytes(down, FP8_DOWN).w : 0;
+        bytes.w = bytes.w > w2 ? bytes.w : w2;
+        tiled = fp8_pad_buffers(bytes, stream, &pads) == 0;
+    }
     const int64_t groups = (int64_t)(tk < a.E ? tk : a.E) * ib;
     const bool wide = !tiled && a.I > 0 && (groups >= kWideGroups || (groups > kSomeGroups && tk > kWideRows * a.E));
     const int bm = tiled ? (tk >= (int64_t)kBigTileRows * a.E && !up.exact ? 256 : 128) : !wide ? 16 : tk <= 8 * a.E ? 16 : tk <= 24 * a.E ? 32 : 64;
@@ -284,6 +291,10 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
         g->row_scale = s.row_scale; g->ld_row_scale = ld;
     }
     if (tiled) {
+        if (pad_up) {
+            rc = pad_fp8_operands(up, FP8_GATE_UP, pads, stream);
+            if (rc) return rc;
+        }
         up.C = s.codes; up.sc_m = ipad;
         rc = launch_gemm_fp8_tile(up, FP8_GATE_UP, stream);
         if (rc) return rc;
@@ -309,8 +320,8 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
     down.a_scale = s.mid_scale;
     down.C = s.y; down.sc_m = hpad;
     if (tiled && pad_down) {
-        rc = pad_fp8_operands(down, FP8_DOWN, stream);
-        if (rc) return rc == TV_E_UNSUPPORTED ? TV_E_NOMEM : rc;
+        rc = pad_fp8_operands(down, FP8_DOWN, pads, stream);
+        if (rc) return rc;
     }
     rc = tiled ? launch_gemm_fp8_tile(down, FP8_DOWN, stream) : wide ? launch_gemm_fp8_wide(down, FP8_DOWN, stream) : launch_gemm_fp8(down, FP8_DOWN, stream);
     if (rc) return rc;

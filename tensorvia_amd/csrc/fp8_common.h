@@ -262,10 +262,18 @@ enum Fp8Mode { FP8_DENSE = 0, FP8_GATE_UP = 1, FP8_DOWN = 2, FP8_SLOT_UP = 3 };
 int launch_gemm_fp8(const Fp8Gemm& g, int mode, hipStream_t stream);
 // BM x BN tiles through LDS.  TV_E_UNSUPPORTED for operands it does not take (fp8_tile_ok).
 bool fp8_tile_ok(const Fp8Gemm& g, int mode);
-// Copies of the operands that are not whole 16-byte rows, zero up to the next 16 bytes, in the stream's padding buffers;
-// g then describes them.  TV_E_UNSUPPORTED (g unchanged) where there is no room, offsets stay too large, or the experts' weights have no one stride.
-bool fp8_pad_ok(const Fp8Gemm& g, int mode); // whether the copies would be taken
-int pad_fp8_operands(Fp8Gemm& g, int mode, hipStream_t stream);
+// Copies of the operands that are not whole 16-byte rows, zero up to the next 16 bytes.  What they need is asked for apart, so that a
+// call of several launches can choose other kernels while nothing is launched.
+bool fp8_pad_ok(const Fp8Gemm& g, int mode); // no: offsets would stay too large, or the experts' weights have no one stride
+struct Fp8PadBytes {
+    size_t a, w; // 0: no copy
+};
+Fp8PadBytes fp8_pad_bytes(const Fp8Gemm& g, int mode);
+struct Fp8Pads {
+    void *a, *w;
+};
+int fp8_pad_buffers(const Fp8PadBytes& bytes, hipStream_t stream, Fp8Pads* pads); // TV_E_UNSUPPORTED: no room
+int pad_fp8_operands(Fp8Gemm& g, int mode, const Fp8Pads& pads, hipStream_t stream); // g then describes the copies
 int launch_gemm_fp8_tile(const Fp8Gemm& g, int mode, hipStream_t stream);
 // The second product of a few tokens from inner rows in fp32, summed over their slots.
 bool fp8_token_ok(const Fp8Gemm& g);

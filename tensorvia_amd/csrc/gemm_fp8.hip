@@ -372,7 +372,12 @@ int launch_gemm_fp8(const Fp8Gemm& g, int mode, hipStream_t stream) {
         if (tile < p.direct && tile < p.wide) {
             Fp8Gemm t = g;
             t.tile_rows = p.tile128 < p.tile256 ? 128 : 256;
-            int rc = fp8_tile_ok(t, mode) ? 0 : pad_fp8_operands(t, mode, stream);
+            int rc = 0;
+            if (!fp8_tile_ok(t, mode)) {
+                Fp8Pads pads;
+                rc = fp8_pad_ok(t, mode) ? fp8_pad_buffers(fp8_pad_bytes(t, mode), stream, &pads) : (int)TV_E_UNSUPPORTED;
+                if (rc == 0) rc = pad_fp8_operands(t, mode, pads, stream);
+            }
             if (rc == 0) rc = launch_gemm_fp8_tile(t, mode, stream);
             if (rc != TV_E_UNSUPPORTED) return rc;
         }

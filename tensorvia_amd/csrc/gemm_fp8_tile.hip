@@ -477,24 +477,37 @@ bool fp8_pad_ok(const Fp8Gemm& g, int mode) {
     return fp8_tile_ok(p, mode) && !(pad_w && mode == FP8_GATE_UP && g.experts > 1 && g.sw_e != 2 * g.sw_g);
 }
 
-int pad_fp8_operands(Fp8Gemm& g, int mode, hipStream_t stream) {
-    if (!fp8_pad_ok(g, mode)) return TV_E_UNSUPPORTED;
+static int64_t pad_a_rows(const Fp8Gemm& g, int mode) { return mode == FP8_GATE_UP ? g.tokens : g.M; }
+static int64_t pad_w_rows(const Fp8Gemm& g, int mode) {
+    return (mode == FP8_DENSE ? 1 : mode == FP8_GATE_UP ? 2 * (int64_t)g.experts : g.experts) * g.N;
+}
+
+Fp8PadBytes fp8_pad_bytes(const Fp8Gemm& g, int mode) {
+    bool pad_a, pad_w;
+    const Fp8Gemm p = padded_fp8(g, mode, &pad_a, &pad_w);
+    return {pad_a ? (size_t)(pad_a_rows(g, mode) * p.K) : 0, pad_w ? (size_t)(pad_w_rows(g, mode) * p.K) : 0};
+}
+
+int fp8_pad_buffers(const Fp8PadBytes& bytes, hipStream_t stream, Fp8Pads* pads) {
+    *pads = Fp8Pads{};
+    if (bytes.w && gemm_pad_workspace(stream, bytes.w, 1, &pads->w) != 0) return TV_E_UNSUPPORTED;
+    if (bytes.a && gemm_pad_workspace(stream, bytes.a, 0, &pads->a) != 0) return TV_E_UNSUPPORTED;
+    return 0;
+}
+
+int pad_fp8_operands(Fp8Gemm& g, int mode, const Fp8Pads& pads, hipStream_t stream) {
     bool pad_a, pad_w;
     Fp8Gemm p = padded_fp8(g, mode, &pad_a, &pad_w);
-    const int64_t P = p.K, a_rows = mode == FP8_GATE_UP ? g.tokens : g.M;
+    const int64_t P = p.K, a_rows = pad_a_rows(g, mode);
     PadJob jobs[2];
     int n = 0;
-    void* ws = nullptr;
     if (pad_a) {
-        if (gemm_pad_workspace(stream, (size_t)(a_rows * P), 0, &ws) != 0) return TV_E_UNSUPPORTED;
-        jobs[n++] = PadJob{g.A, ws, a_rows, a_rows, g.sa_m, 0, g.K, P};
-        p.A = static_cast<const uint8_t*>(ws);
+        jobs[n++] = PadJob{g.A, pads.a, a_rows, a_rows, g.sa_m, 0, g.K, P};
+        p.A = static_cast<const uint8_t*>(pads.a);
     }
     if (pad_w) {
-        const int64_t mats = mode == FP8_DENSE ? 1 : mode == FP8_GATE_UP ? 2 * g.experts : g.experts;
-        if (gemm_pad_workspace(stream, (size_t)(mats * g.N * P), 1, &ws) != 0) return TV_E_UNSUPPORTED;
-        jobs[n++] = PadJob{g.W, ws, g.N, mats * g.N, g.sw_n, mode == FP8_GATE_UP ? g.sw_g : g.sw_e, g.K, P};
-        p.W = static_cast<const uint8_t*>(ws);
+        jobs[n++] = PadJob{g.W, pads.w, g.N, pad_w_rows(g, mode), g.sw_n, mode == FP8_GATE_UP ? g.sw_g : g.sw_e, g.K, P};
+        p.W = static_cast<const uint8_t*>(pads.w);
     }
     g = p;
     return n ? launch_pad_rows(jobs, n, 1, stream) : 0;
