@@ -18,13 +18,13 @@ namespace tvk {
 //  FP8_GATE_UP  rows of one expert, gathered through row_token; both halves of W1, C = silu(gate) * up in fp32;
 //  FP8_SLOT_UP  the same without a plan: a tile is one slot;
 //  FP8_DOWN     rows of one expert in the plan's order, times their routing weight, in fp32.
-template <typename TC, int MODE, int MT, int KW, int U, int ROWS>
+//  EXACT: exact products of a block (mfma_fp8_exact), for fp32 results, and for the inner rows, which are rounded to e4m3 next: an error
+//  of 1.5e-5 moves one value in two thousand to the other code beside it, which shows where the rows are few.  (W's bytes
+//  bound the call either way.)
+template <typename TC, int MODE, bool EXACT, int MT, int KW, int U, int ROWS>
 __global__ __launch_bounds__(64 * KW) void gemm_fp8_direct_kernel(Fp8Gemm g) {
     constexpr int NG = MODE == FP8_GATE_UP || MODE == FP8_SLOT_UP ? 2 : 1;
     constexpr int PITCH = 17; // floats per row of 16 sums
-    // Exact products for fp32 results, and for the inner rows, which are rounded to e4m3 next: an error of 1.5e-5 moves one value
-    // in two thousand to the other code beside it, which shows where the rows are few.  (W's bytes bound the call either way.)
-    constexpr bool kExact = (MODE == FP8_DENSE && __is_same(TC, float)) || NG == 2;
     __shared__ float sums[KW][NG][MT * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, grp = lane >> 4;
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * KW) void gemm_fp8_direct_kernel(Fp8Gemm g) {
     // used: uniform; a select, not a branch, so that the loads stay ahead of it (and a NaN that is not used does not count).
     auto multiply = [&](const i32x8& w, const i32x8& x, float s, f32x4& sum, bool used) {
         f32x4 t;
-        if constexpr (kExact) t = mfma_fp8_exact(w, x);
+        if constexpr (EXACT) t = mfma_fp8_exact(w, x);
         else t = mfma_fp8(w, x);
 #pragma unroll
         for (int q = 0; q < 4; ++q) sum[q] = used ? __builtin_fmaf(s, t[q], sum[q]) : sum[q];
@@ -229,7 +229,10 @@ __global__ __launch_bounds__(64 * kTokenWaves) void gemm_fp8_token_kernel(Fp8Gem
         for (int u = 0; u < kTokenU; ++u) {
             const int q = q0 + u * kTokenWaves, qc = min(q, total - 1);
             const char* x = codes + qc * TV_FP8_BLOCK + grp * kLaneStep<ROWS>;
-            const f32x4 t = mfma_fp8(w[u].f.get(w[u].shift), join(*reinterpret_cast<const u32x4*>(x), *reinterpret_cast<const u32x4*>(x + kSecondHalf<ROWS>)));
+            const i32x8 wq = w[u].f.get(w[u].shift), xq = join(*reinterpret_cast<const u32x4*>(x), *reinterpret_cast<const u32x4*>(x + kSecondHalf<ROWS>));
+            f32x4 t;
+            if constexpr (__is_same(TC, float)) t = mfma_fp8_exact(wq, xq);
+            else t = mfma_fp8(wq, xq);
             const float s = scales[qc] * w[u].s;
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] = w[u].used ? __builtin_fmaf(s, t[i], acc[i]) : acc[i];
@@ -274,7 +277,7 @@ int launch_gemm_fp8_token(const Fp8Gemm& g, const float* mid, int64_t ld, int to
     }
 }
 
-template <typename TC, int MODE, int MT, int KW, int U> static int direct(const Fp8Gemm& g, bool fast, hipStream_t stream) {
+template <typename TC, int MODE, bool EXACT, int MT, int KW, int U> static int direct(const Fp8Gemm& g, bool fast, hipStream_t stream) {
     const int64_t mt = MODE == FP8_DENSE ? ((int64_t)g.M + 16 * MT - 1) / (16 * MT) : MODE == FP8_SLOT_UP ? g.M : g.max_tiles;
     const int64_t nt = ((int64_t)g.N + 15) / 16;
     // The grid's rows are limited to 65535, its threads to 2^32.
@@ -284,8 +287,8 @@ template <typename TC, int MODE, int MT, int KW, int U> static int direct(const 
         Fp8Gemm p = g;
         p.first_tile = (int32_t)y;
         const dim3 grid((unsigned)nt, (unsigned)(mt - y < rows ? mt - y : rows));
-        if (fast) hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, MT, KW, U, FP8_ALIGNED>), grid, dim3(64 * KW), 0, stream, p);
-        else hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, MT, KW, U, FP8_ANY>), grid, dim3(64 * KW), 0, stream, p);
+        if (fast) hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ALIGNED>), grid, dim3(64 * KW), 0, stream, p);
+        else hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ANY>), grid, dim3(64 * KW), 0, stream, p);
         const int rc = hipGetLastError();
         if (rc) return rc;
     }
@@ -294,16 +297,17 @@ template <typename TC, int MODE, int MT, int KW, int U> static int direct(const 
 
 // One block of k in flight per wave up to 16 blocks, four beyond.  us in bf16, one row, one block in flight / four:
 // [1024 -> 4096] 2.8 / 4.5, [2048 -> 11008] 6.3 / 9.4, [4096 -> 4096] 5.5 / 5.4, [4096 -> 11008] 10.4 / 9.9.
-template <typename TC, int MODE> static int direct_u(const Fp8Gemm& g, bool fast, hipStream_t stream) {
-    if (g.K <= 16 * TV_FP8_BLOCK) return direct<TC, MODE, 1, 8, 1>(g, fast, stream);
-    return direct<TC, MODE, 1, 8, 4>(g, fast, stream);
+template <typename TC, int MODE, bool EXACT> static int direct_u(const Fp8Gemm& g, bool fast, hipStream_t stream) {
+    if (g.K <= 16 * TV_FP8_BLOCK) return direct<TC, MODE, EXACT, 1, 8, 1>(g, fast, stream);
+    return direct<TC, MODE, EXACT, 1, 8, 4>(g, fast, stream);
 }
 
 // rows: of a workgroup.
 template <typename TC> static int dense(const Fp8Gemm& g, bool fast, int rows, hipStream_t stream) {
-    if (rows == 16) return direct_u<TC, FP8_DENSE>(g, fast, stream);
-    if (rows == 32) return direct<TC, FP8_DENSE, 2, 8, 1>(g, fast, stream);
-    return direct<TC, FP8_DENSE, 4, 8, 1>(g, fast, stream);
+    constexpr bool exact = __is_same(TC, float);
+    if (rows == 16) return direct_u<TC, FP8_DENSE, exact>(g, fast, stream);
+    if (rows == 32) return direct<TC, FP8_DENSE, exact, 2, 8, 1>(g, fast, stream);
+    return direct<TC, FP8_DENSE, exact, 4, 8, 1>(g, fast, stream);
 }
 
 // What a dense product of more than 16 rows takes on each kernel, in us, and the kernel that takes least.  Fitted to bf16
@@ -361,9 +365,9 @@ static Fp8Price price(const Fp8Gemm& g, bool fast) {
 
 int launch_gemm_fp8(const Fp8Gemm& g, int mode, hipStream_t stream) {
     const bool fast = fast_rows(g.A, g.M, g.sa_m, g.K) && fast_rows(g.W, g.N, g.sw_n, g.K) && g.sw_e % 16 == 0 && g.sw_g % 16 == 0;
-    if (mode == FP8_GATE_UP) return direct_u<float, FP8_GATE_UP>(g, fast, stream);
-    if (mode == FP8_SLOT_UP) return direct_u<float, FP8_SLOT_UP>(g, fast, stream);
-    if (mode == FP8_DOWN) return direct_u<float, FP8_DOWN>(g, fast, stream);
+    if (mode == FP8_GATE_UP) return direct_u<float, FP8_GATE_UP, true>(g, fast, stream);
+    if (mode == FP8_SLOT_UP) return direct_u<float, FP8_SLOT_UP, true>(g, fast, stream);
+    if (mode == FP8_DOWN) return g.dtype_c == TV_FLOAT32 ? direct_u<float, FP8_DOWN, true>(g, fast, stream) : direct_u<float, FP8_DOWN, false>(g, fast, stream);
     int rows = 16;
     if (g.M > 16 && g.K > 0) {
         const Fp8Price p = price(g, fast);

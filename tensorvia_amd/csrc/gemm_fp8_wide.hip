@@ -15,12 +15,11 @@
 
 namespace tvk {
 
-template <int MODE_, typename TC_, int MT_, int ROWS_> struct Fp8Wide {
+template <int MODE_, typename TC_, bool EXACT_, int MT_, int ROWS_> struct Fp8Wide {
     using TC = TC_;
     static constexpr int MODE = MODE_, MT = MT_, BM = 16 * MT_, NG = MODE_ == FP8_GATE_UP ? 2 : 1;
     static constexpr int ROWS = ROWS_;
-    // Exact products of a block, as the direct kernel's.
-    static constexpr bool EXACT = MODE_ == FP8_GATE_UP || (MODE_ == FP8_DENSE && __is_same(TC_, float));
+    static constexpr bool EXACT = EXACT_; // exact products of a block, as the direct kernel's
     static constexpr int WAVES = 8, THREADS = 512;
     static constexpr int KC = 2;                         // blocks of k per chunk
     static constexpr int PITCH = KC * 128 + 16;          // bytes of a row's chunk in LDS: 16 rows on distinct banks
@@ -326,26 +325,26 @@ template <class C> static int run_wide(const Fp8Gemm& g, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int MODE, typename TC, int ROWS> static int wide_rows(const Fp8Gemm& g, hipStream_t stream) {
+template <int MODE, typename TC, bool EXACT, int ROWS> static int wide_rows(const Fp8Gemm& g, hipStream_t stream) {
     const int rows = MODE == FP8_DENSE ? g.M : g.tile_rows;
     if constexpr (MODE != FP8_DENSE)
-        if (rows <= 16) return run_wide<Fp8Wide<MODE, TC, 1, ROWS>>(g, stream);
-    if (rows <= 32) return run_wide<Fp8Wide<MODE, TC, 2, ROWS>>(g, stream);
-    return run_wide<Fp8Wide<MODE, TC, 4, ROWS>>(g, stream);
+        if (rows <= 16) return run_wide<Fp8Wide<MODE, TC, EXACT, 1, ROWS>>(g, stream);
+    if (rows <= 32) return run_wide<Fp8Wide<MODE, TC, EXACT, 2, ROWS>>(g, stream);
+    return run_wide<Fp8Wide<MODE, TC, EXACT, 4, ROWS>>(g, stream);
 }
-template <int MODE, typename TC> static int wide(const Fp8Gemm& g, hipStream_t stream) {
+template <int MODE, typename TC, bool EXACT> static int wide(const Fp8Gemm& g, hipStream_t stream) {
     const bool fast = fast_rows(g.A, MODE == FP8_GATE_UP ? g.tokens : g.M, g.sa_m, g.K) && fast_rows(g.W, g.N, g.sw_n, g.K) &&
                       g.sw_e % 16 == 0 && g.sw_g % 16 == 0;
-    return fast ? wide_rows<MODE, TC, FP8_ALIGNED>(g, stream) : wide_rows<MODE, TC, FP8_ANY>(g, stream);
+    return fast ? wide_rows<MODE, TC, EXACT, FP8_ALIGNED>(g, stream) : wide_rows<MODE, TC, EXACT, FP8_ANY>(g, stream);
 }
 
 int launch_gemm_fp8_wide(const Fp8Gemm& g, int mode, hipStream_t stream) {
-    if (mode == FP8_GATE_UP) return wide<FP8_GATE_UP, uint8_t>(g, stream);
-    if (mode == FP8_DOWN) return wide<FP8_DOWN, float>(g, stream);
+    if (mode == FP8_GATE_UP) return wide<FP8_GATE_UP, uint8_t, true>(g, stream);
+    if (mode == FP8_DOWN) return g.dtype_c == TV_FLOAT32 ? wide<FP8_DOWN, float, true>(g, stream) : wide<FP8_DOWN, float, false>(g, stream);
     switch (g.dtype_c) {
-        case TV_BFLOAT16: return wide<FP8_DENSE, __bf16>(g, stream);
-        case TV_FLOAT16: return wide<FP8_DENSE, _Float16>(g, stream);
-        default: return wide<FP8_DENSE, float>(g, stream);
+        case TV_BFLOAT16: return wide<FP8_DENSE, __bf16, false>(g, stream);
+        case TV_FLOAT16: return wide<FP8_DENSE, _Float16, false>(g, stream);
+        default: return wide<FP8_DENSE, float, true>(g, stream);
     }
 }
 
