@@ -231,6 +231,7 @@ struct Fp8Gemm {
     int32_t experts;
     int32_t max_tiles;
     int32_t first_tile;         // of this launch, where the tiles need several
+    int32_t first_col;          // of this launch, where the columns need several
     int32_t tokens;             // rows that row_token names
     int32_t tile_rows;          // rows of the plan's tiles
     int32_t exact;              // gate-and-up product in tiles: exact products within a block

@@ -28,13 +28,13 @@ __global__ __launch_bounds__(64 * KW) void gemm_fp8_direct_kernel(Fp8Gemm g) {
     __shared__ float sums[KW][NG][MT * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, grp = lane >> 4;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = g.first_col + (int)blockIdx.x * 16;
     int m0, m1, expert = 0; // rows of this tile
     if constexpr (MODE == FP8_DENSE) {
         m0 = (g.first_tile + (int)blockIdx.y) * MT * 16;
         m1 = min(g.M, m0 + MT * 16);
     } else if constexpr (MODE == FP8_SLOT_UP) {
-        m0 = blockIdx.y; // a slot is its own row and tile
+        m0 = g.first_tile + (int)blockIdx.y; // a slot is its own row and tile
         m1 = m0 + 1;
         expert = g.ids[m0];
         if ((unsigned)expert >= (unsigned)g.experts) return;
@@ -281,17 +281,18 @@ template <typename TC, int MODE, bool EXACT, int MT, int KW, int U> static int d
     const int64_t mt = MODE == FP8_DENSE ? ((int64_t)g.M + 16 * MT - 1) / (16 * MT) : MODE == FP8_SLOT_UP ? g.M : g.max_tiles;
     const int64_t nt = ((int64_t)g.N + 15) / 16;
     // The grid's rows are limited to 65535, its threads to 2^32.
-    const int64_t room = (((int64_t)1 << 32) / (64 * KW) - 1) / nt, rows = room < 32768 ? room : 32768;
-    if (rows < 1 || (MODE == FP8_SLOT_UP && mt > rows)) return TV_E_SHAPE; // over 2^27 columns
-    for (int64_t y = 0; y < mt; y += rows) {
-        Fp8Gemm p = g;
-        p.first_tile = (int32_t)y;
-        const dim3 grid((unsigned)nt, (unsigned)(mt - y < rows ? mt - y : rows));
-        if (fast) hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ALIGNED>), grid, dim3(64 * KW), 0, stream, p);
-        else hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ANY>), grid, dim3(64 * KW), 0, stream, p);
-        const int rc = hipGetLastError();
-        if (rc) return rc;
-    }
+    const int64_t room = ((int64_t)1 << 32) / (64 * KW) - 1, cols = nt < room ? nt : room, rows = room / cols < 32768 ? room / cols : 32768;
+    for (int64_t x = 0; x < nt; x += cols)
+        for (int64_t y = 0; y < mt; y += rows) {
+            Fp8Gemm p = g;
+            p.first_col = (int32_t)(x * 16);
+            p.first_tile = (int32_t)y;
+            const dim3 grid((unsigned)(nt - x < cols ? nt - x : cols), (unsigned)(mt - y < rows ? mt - y : rows));
+            if (fast) hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ALIGNED>), grid, dim3(64 * KW), 0, stream, p);
+            else hipLaunchKernelGGL((gemm_fp8_direct_kernel<TC, MODE, EXACT, MT, KW, U, FP8_ANY>), grid, dim3(64 * KW), 0, stream, p);
+            const int rc = hipGetLastError();
+            if (rc) return rc;
+        }
     return 0;
 }
 

@@ -18,3 +18,20 @@ def test_gemm_scales_of_distant_blocks(hip, m, n, k):
     far = torch.empty((blocks - 1) * step + m, device="cuda").as_strided((m, blocks), (1, step))
     far.copy_(a_scale)
     check_gemm(tv.gemm_fp8(a, far, w, w_scale), a, a_scale, w, w_scale, "bf16")
+
+
+@pytest.mark.parametrize("m,k", [(1, 5), (2, 16), (16, 3)])
+def test_gemm_of_more_columns_than_a_grid(hip, m, k):
+    """2^27 columns and more, which the workgroups of 16 columns take in several launches: the first ones, those around the
+    launches' seam and the last ones."""
+    n = (1 << 27) + 1003
+    a, a_scale = ref.rand_rows(m, k, 23)
+    g = torch.Generator("cuda").manual_seed(24)
+    w = torch.randint(0, 0x78, (n, k), dtype=torch.uint8, device="cuda", generator=g)
+    w[::3] |= 0x80
+    w = w.view(torch.float8_e4m3fn)
+    w_scale = 0.5 + torch.rand(ref.up(n), 1, device="cuda", generator=g)
+    c = tv.gemm_fp8(a, a_scale, w, w_scale)
+    for first in (0, (1 << 27) - 384, n // 128 * 128 - 256):
+        last = min(n, first + 700)
+        check_gemm(c[:, first:last], a, a_scale, w[first:last], w_scale[first // 128:ref.up(last)], "bf16")
