@@ -149,7 +149,8 @@ __device__ inline void store_codes8(uint8_t* p, int64_t n, const float (&v)[8], 
     }
 }
 
-// Most workgroups these launchers start (grid x block stays below 2^32 threads); kernels loop where there is more work.
+// Most workgroups these launchers start (grid x block stays below 2^32 threads); kernels loop where there is more work, or
+// are launched again.
 constexpr int64_t kMaxGrid = 1 << 20;
 
 // How the rows of a product's operands lie: whole 16-byte chunks at 16-byte aligned addresses, or anything.  A lane holds 32

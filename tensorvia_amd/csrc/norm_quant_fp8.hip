@@ -38,9 +38,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(tv_quantize_fp8_args
 // with 256 threads and 8 steps 32.8; four blocks side by side in a workgroup, whole rows of 1 KB but
 // half the waves on a CU, 34.6).
 template <typename T, bool SHORT>
-__global__ __launch_bounds__(512) void quantize_tiles_kernel(tv_quantize_fp8_args a, int64_t kb) {
+__global__ __launch_bounds__(512) void quantize_tiles_kernel(tv_quantize_fp8_args a, int64_t kb, int64_t first) {
     __shared__ unsigned part[8];
-    const int64_t mb = blockIdx.x / kb, b = blockIdx.x - mb * kb;
+    const int64_t at = first + blockIdx.x, mb = at / kb, b = at - mb * kb;
     const int64_t k = b * TV_FP8_BLOCK + (threadIdx.x & 15) * 8, left = a.K - k;
     const int64_t m0 = mb * TV_FP8_BLOCK + (threadIdx.x >> 4);
     Eight<T, SHORT> x[4];
@@ -80,8 +80,12 @@ template <typename T, bool SHORT> static int quantize(const tv_quantize_fp8_args
         hipLaunchKernelGGL((quantize_rows_kernel<T, SHORT>), dim3((unsigned)(wgs < kMaxGrid ? wgs : kMaxGrid)), dim3(256), 0, stream, a, n, kb);
     } else {
         const int64_t n = (a.M + TV_FP8_BLOCK - 1) / TV_FP8_BLOCK * kb;
-        if (n > 0x7fffff) return TV_E_SHAPE; // 2^23 blocks: 2^37 elements, beyond any device's memory
-        hipLaunchKernelGGL((quantize_tiles_kernel<T, SHORT>), dim3((unsigned)n), dim3(512), 0, stream, a, kb);
+        for (int64_t first = 0; first < n; first += kMaxGrid) {
+            hipLaunchKernelGGL((quantize_tiles_kernel<T, SHORT>), dim3((unsigned)(n - first < kMaxGrid ? n - first : kMaxGrid)), dim3(512), 0, stream, a, kb, first);
+            const int rc = hipGetLastError();
+            if (rc) return rc;
+        }
+        return 0;
     }
     return hipGetLastError();
 }

@@ -4,7 +4,7 @@ import torch
 
 import tensorvia_amd as tv
 from tests import fp8_ref as ref
-from tests.test_fp8_gpu import check_gemm
+from tests.test_fp8_gpu import check_codes, check_gemm
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,17 @@ def test_gemm_of_more_columns_than_a_grid(hip, m, k):
     for first in (0, (1 << 27) - 384, n // 128 * 128 - 256):
         last = min(n, first + 700)
         check_gemm(c[:, first:last], a, a_scale, w[first:last], w_scale[first // 128:ref.up(last)], "bf16")
+
+
+def test_quantize_more_blocks_than_a_grid(hip):
+    """2^23 blocks of weights and one, of one column: the first ones, those around the launches' seams and the last, short one."""
+    m = (1 << 30) + 57
+    x = torch.zeros(m, 1, dtype=torch.bfloat16, device="cuda")
+    seam = 128 << 20
+    windows = [(first, min(m, first + 1024)) for first in (0, seam - 512, 7 * seam - 512, (1 << 30) - 512)]
+    g = torch.Generator("cuda").manual_seed(25)
+    for first, last in windows:
+        x[first:last] = torch.randn(last - first, 1, device="cuda", generator=g)
+    q, scale = tv.quantize_fp8(x, 128)
+    for first, last in windows:
+        check_codes(q[first:last], scale[first // 128:ref.up(last)], x[first:last].double(), 128, 0.0)
