@@ -175,6 +175,9 @@ constexpr int kTileRows = 22, kExactTileRows = 28, kPadTileRows = 100, kPadDownT
 // rows) 50 / 55; [100,1003,503,16,4] (64, 25 rows) 37 / 35; [110,1024,512,8,2] (32, 27 rows) 27 / 23.
 constexpr int kWideGroups = 128, kSomeGroups = 64, kWideRows = 13;
 
+// Workgroups of the tiles' and the wide kernels' grids, 512 threads each.
+constexpr int64_t kTileGrid = (int64_t)1 << 22, kWideGrid = (int64_t)1 << 23;
+
 // Tokens up to which their slots may go without a plan.
 constexpr int kFewTokens = 4;
 
@@ -212,7 +215,7 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
     down.ids = up.ids = a.ids;
     down.route_w = a.weights;
     down.dtype_c = a.dtype_c;
-    if ((a.T == 1 || (a.T <= kFewTokens && 2 * tk <= a.E)) && a.I > 0 && fp8_token_ok(down)) {
+    if ((a.T == 1 || (a.T <= kFewTokens && 2 * tk <= a.E)) && a.I > 0 && fp8_token_ok(down, (int)a.T)) {
         void* mid = nullptr;
         const int rc = experts_workspace(stream, (size_t)tk * ipad * 4, &mid);
         if (rc) return rc;
@@ -234,6 +237,12 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
     up.exact = a.dtype_c != TV_BFLOAT16;
     bool tiled = tk >= (int64_t)(pad_up ? kPadTileRows : pad_down ? kPadDownTileRows : up.exact ? kExactTileRows : kTileRows) * a.E && a.dtype_c != TV_FLOAT32 && a.I > 0;
     tiled = tiled && (!pad_up || fp8_pad_ok(up, FP8_GATE_UP)) && (!pad_down || fp8_pad_ok(down, FP8_DOWN));
+    // Rows of up to `bm` make at most this many tiles.  A grid's threads are limited: calls beyond take the next kernel, the direct one
+    // runs in several launches.
+    const auto tiles_of = [&](int64_t bm) { return (tk < a.E ? tk : a.E) + tk / bm; };
+    const auto grid_ok = [&](int64_t bm, int64_t most) { return tiles_of(bm) * (hb > ib ? hb : ib) <= most - 8; };
+    const int tile_rows = tk >= (int64_t)kBigTileRows * a.E && !up.exact ? 256 : 128;
+    tiled = tiled && grid_ok(tile_rows, kTileGrid);
     // One buffer holds W1's copy, then W2's.  Without room for it the other kernels run.
     Fp8Pads pads{};
     if (tiled && (pad_up || pad_down)) {
@@ -243,9 +252,10 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
         tiled = fp8_pad_buffers(bytes, stream, &pads) == 0;
     }
     const int64_t groups = (int64_t)(tk < a.E ? tk : a.E) * ib;
-    const bool wide = !tiled && a.I > 0 && (groups >= kWideGroups || (groups > kSomeGroups && tk > kWideRows * a.E));
-    const int bm = tiled ? (tk >= (int64_t)kBigTileRows * a.E && !up.exact ? 256 : 128) : !wide ? 16 : tk <= 8 * a.E ? 16 : tk <= 24 * a.E ? 32 : 64;
-    const int max_tiles = (tk < a.E ? tk : a.E) + tk / bm;
+    const int wide_rows = tk <= 8 * a.E ? 16 : tk <= 24 * a.E ? 32 : 64;
+    const bool wide = !tiled && a.I > 0 && (groups >= kWideGroups || (groups > kSomeGroups && tk > kWideRows * a.E)) && grid_ok(wide_rows, kWideGrid);
+    const int bm = tiled ? tile_rows : wide ? wide_rows : 16;
+    const int max_tiles = (int)tiles_of(bm);
 
     ExpertScratch s{};
     size_t need = 0;

@@ -278,7 +278,7 @@ int fp8_pad_buffers(const Fp8PadBytes& bytes, hipStream_t stream, Fp8Pads* pads)
 int pad_fp8_operands(Fp8Gemm& g, int mode, const Fp8Pads& pads, hipStream_t stream); // g then describes the copies
 int launch_gemm_fp8_tile(const Fp8Gemm& g, int mode, hipStream_t stream);
 // The second product of a few tokens from inner rows in fp32, summed over their slots.
-bool fp8_token_ok(const Fp8Gemm& g);
+bool fp8_token_ok(const Fp8Gemm& g, int tokens);
 int launch_gemm_fp8_token(const Fp8Gemm& g, const float* mid, int64_t ld, int tokens, hipStream_t stream);
 // 16 to 64 rows and 128 columns a workgroup, W straight from memory.
 int launch_gemm_fp8_wide(const Fp8Gemm& g, int mode, hipStream_t stream);

@@ -257,8 +257,9 @@ static size_t token_lds(const Fp8Gemm& g) {
     return bytes > kTokenWaves * 64 ? bytes : kTokenWaves * 64;
 }
 
-bool fp8_token_ok(const Fp8Gemm& g) {
-    return token_lds(g) <= 64 * 1024;
+// tokens: rows of the grid, whose threads are limited to 2^32.
+bool fp8_token_ok(const Fp8Gemm& g, int tokens) {
+    return token_lds(g) <= 64 * 1024 && ((int64_t)g.N + 15) / 16 * tokens < ((int64_t)1 << 32) / (64 * kTokenWaves);
 }
 
 int launch_gemm_fp8_token(const Fp8Gemm& g, const float* mid, int64_t ld, int tokens, hipStream_t stream) {

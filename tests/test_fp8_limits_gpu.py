@@ -4,7 +4,8 @@ import torch
 
 import tensorvia_amd as tv
 from tests import fp8_ref as ref
-from tests.test_fp8_gpu import check_codes, check_gemm
+from tests.test_experts_gpu import check as check_experts
+from tests.test_fp8_gpu import DT, check_codes, check_gemm
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,49 @@ def test_quantize_more_blocks_than_a_grid(hip):
     q, scale = tv.quantize_fp8(x, 128)
     for first, last in windows:
         check_codes(q[first:last], scale[first // 128:ref.up(last)], x[first:last].double(), 128, 0.0)
+
+
+def shared_experts(t, h, i, e, k, seed):
+    """Arguments of a layer whose experts share one pair of codes (strides of 0) under scales of their own."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    a, a_scale = ref.rand_rows(t, h, seed)
+    w1, w2 = (ref.rand_weights(shape, seed + 1)[0].expand(e, *shape[1:]) for shape in ((1, 2, i, h), (1, h, i)))
+    w1_scale = (0.02 / 107) * torch.exp(0.2 * torch.randn(e, 2, ref.up(i), ref.up(h), device="cuda", generator=g))
+    w2_scale = (0.02 / 107) * torch.exp(0.2 * torch.randn(e, ref.up(h), ref.up(i), device="cuda", generator=g))
+    weights, ids = torch.softmax(torch.randn(t, e, device="cuda", generator=g), -1).topk(k, -1)
+    return [a, a_scale, w1, w1_scale, w2, w2_scale, (weights / weights.sum(-1, keepdim=True)).contiguous(), ids.to(torch.int32)]
+
+
+def check_tokens(got, args, tokens, out):
+    tokens = torch.tensor(tokens, device="cuda")
+    part = [x.view(torch.uint8)[tokens].view(x.dtype) if x.dtype == torch.float8_e4m3fn else x[tokens].contiguous() for x in args[:2]]
+    check_experts(got[tokens], part + args[2:6] + [args[6][tokens], args[7][tokens]], out)
+
+
+@pytest.mark.parametrize("t,i,e,k,out", [(2816, 448_000, 1024, 8, "bf16"), (1024, 1_000_000, 1024, 1, "f32")])
+def test_experts_of_more_workgroups_than_a_grid(hip, t, i, e, k, out):
+    """Widths at which the tiles' grid, and that of the workgroups of 128 columns, would hold too many threads."""
+    args = shared_experts(t, 16, i, e, k, 26)
+    check_tokens(tv.experts_fp8(*args, out_dtype=tv.torch_to_tv(DT[out])), args, [0, t // 2, t - 1], out)
+
+
+def test_one_token_of_more_columns_than_a_grid(hip):
+    """A row of 2^26 elements and more through one expert.  Its first 1024 elements are not zero; the results' first, middle and
+    last ones."""
+    h, i, part = (1 << 26) + 2048, 16, 1024
+    g = torch.Generator("cuda").manual_seed(27)
+
+    def codes(*shape):
+        w = torch.randint(0, 0x70, shape, dtype=torch.uint8, device="cuda", generator=g)
+        w[..., ::3] |= 0x80
+        return w.view(torch.float8_e4m3fn)
+    a = torch.zeros(1, h, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    a[:, :part] = codes(1, part)
+    w1, w2 = codes(1, 2, i, h), codes(1, h, i)
+    scales = [1e-3 + 1e-3 * torch.rand(shape, device="cuda", generator=g) for shape in ((1, ref.up(h)), (1, 2, 1, ref.up(h)), (1, ref.up(h), 1))]
+    weights, ids = torch.full((1, 1), 0.5, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    got = tv.experts_fp8(a, scales[0], w1, scales[1], w2, scales[2], weights, ids)
+    for first in (0, 1 << 25, h - part):
+        block = slice(first // 128, (first + part) // 128)
+        check_experts(got[:, first:first + part], [a[:, :part], scales[0][:, :8], w1[..., :part], scales[1][..., :8], w2[:, first:first + part],
+                                                   scales[2][:, block], weights, ids], "bf16")
