@@ -9,9 +9,9 @@
 // A round of the choice: the largest value (as order-preserving bits, one maximum), then the lowest index that
 // has it (one minimum).  Scores wait in LDS for the k indices.
 //
-// The choice must not depend on the order of a sum: the softmax's denominator is summed in 64 bits and
-// rounded to fp32 once, so any order gives the same scores.  (Up to 1024 terms of 24 bits in [0, 1], the
-// largest 1: the 53-bit sum is exact down to terms of 2^-29 and off by 2^-50 in all below.)
+// The softmax's denominator is summed in 64 bits and rounded to fp32 once.  Up to 1024 terms in [0, 1], the largest 1: in any order
+// the 64-bit sum is off by at most 1024 * 2^-53 = 2^-43 of itself, so two orders (16 lanes or 64 a token) give scores that differ only
+// where the sum lies that close to the middle between two fp32 numbers: one sum in 2^18 at the very most.
 #include "fp8_common.h"
 
 namespace tvk {
