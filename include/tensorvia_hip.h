@@ -265,8 +265,8 @@ int tv_hip_rms_norm_fp8(const tv_rms_norm_fp8_args* args, void* hip_stream);
  * sum on random codes, 3e-5 to 6e-5 where one value of a row is 30 to 448 times the others (half an ulp of a
  * 16-bit result is 2e-3 or 2.4e-4 of it, or more).  Split products add their parts in one order: the same call
  * gives the same bits.
- * Needs no workspace, but uses the stream's, where it can be had, for the partial sums of split products (32 MiB at most) and, from
- * about a hundred rows on, for copies of operands whose rows are not whole 16-byte chunks at 16-byte aligned addresses
+ * Needs no workspace, but uses the stream's, where it can be had, for the partial sums of split products (32 MiB at most) and, in
+ * large products, for copies of operands whose rows are not whole 16-byte chunks at 16-byte aligned addresses
  * (M and N rows of K rounded up to 16). */
 typedef struct tv_gemm_fp8_args {
     int32_t dtype_c, flags; /* flags: reserved, must be 0 */
@@ -305,7 +305,7 @@ int tv_hip_route(const tv_route_args* args, void* hip_stream);
 
 /* A layer of experts on quantised rows: for every token t and slot j < k with expert e = ids[t, j],
  *   h = silu(x_t W1[e, 0]^T) * (x_t W1[e, 1]^T)      [I], fp32, quantised in 1 x 128 blocks,
- *   C[t] = sum_j weights[t, j] * (h W2[e]^T)          [H], summed in fp32 in slot order, rounded to dtype_c,
+ *   C[t] = sum_j weights[t, j] * (h W2[e]^T)          [H], summed in fp32 in a fixed order, rounded to dtype_c,
  * x_t the row of A [T, H]; W1 [E, 2, I, H] (gate, up) and W2 [E, H, I] in 128 x 128 blocks, scales dense
  * [E, 2, ceil(I/128), ceil(H/128)] and [E, ceil(H/128), ceil(I/128)].  Slots with an id below 0 or not
  * below E have no expert and add nothing; a token without experts gets a row of zeros.
