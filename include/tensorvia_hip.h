@@ -312,7 +312,8 @@ int tv_hip_route(const tv_route_args* args, void* hip_stream);
  * E <= TV_ROUTE_MAX_EXPERTS, k <= 64, T * k below 2^31 - 2^20.
  * Large calls (22 slots an expert and more, a 16-bit result) keep each slot's product, until the sum, as
  * fp16 with a power of two per 64 columns: a rounding to 11 bits before the one to dtype_c.  Block sums
- * of the first product are exact (see tv_gemm_fp8_args), but in large calls with a BFLOAT16 result, whose two products both
+ * of the first product are exact (see tv_gemm_fp8_args), but in such calls of 8192 slots and more with a BFLOAT16
+ * result, whose two products both
  * use the 8-bit instructions; those of the second product are exact for a FLOAT32 result and the 8-bit instructions'
  * for 16-bit ones.
  * Needs a workspace per stream, grown as tv_hip_gemm's is, of at most 5 I' + 4 H' + I' / 32 + 13 bytes a slot, I' = I

@@ -167,6 +167,13 @@ struct ExpertScratch {
 // rows 735 / 583, 96 rows 734 / 700, 128 rows 744 / 872; W2 alone, [T,2048], 16 experts of 1001, 75 rows 64 / 66.  64 rows: 333 in
 // tiles of 256, 338 of 128.
 constexpr int kTileRows = 22, kExactTileRows = 28, kPadTileRows = 100, kPadDownTileRows = 72, kBigTileRows = 64;
+// Slots from which tiles with a bf16 result go without exact sums.  A moved code of a row's largest value changes its result by a
+// fourteenth, and with few rows a few of them decide the error: relative to the plain form's, over 40 calls each of 8 experts, median and
+// largest, I 128 / H 512 and I 512 / H 1536: 240 slots 1.12, 4.3 and 1.24, 2.9; 1000 slots 1.18, 2.3 and 1.21, 1.8; 5600
+// slots 1.22, 1.5 and 1.24, 1.32; 11200 slots 1.25, 1.42 and 1.24, 1.34.  Exact sums below that: us, exact / not, [T,4096], 64 experts
+// of 1376, k = 8: 256 tokens 290 / 274, 512 367 / 324, 1000 444 / 388; [T,1024], 8 of 512, k = 2: 110 tokens 25 / 29, 1500 42 / 47;
+// [4000,4096], 8 of 1376, k = 2: 303 / 226.
+constexpr int kExactSlots = 8192;
 // Below those, workgroups of 128 columns read an expert's weights once for up to 64 rows, workgroups of 16 columns and 16
 // rows read them for every 16 rows but are eight times as many.  The first run where at most one workgroup per expert
 // and 128 of I makes at least kWideGroups, or with more than kWideRows rows an expert more than kSomeGroups.  us, wide /
@@ -232,9 +239,9 @@ static int run_experts(const tv_experts_fp8_args& a, hipStream_t stream) {
     const bool pad_up = !fp8_tile_ok(up, FP8_GATE_UP), pad_down = !fp8_tile_ok(down, FP8_DOWN);
     // The inner rows are rounded to e4m3: the 8-bit instructions' error of 1.5e-5 moves one value in two thousand to the other code
     // beside it, together 1.2e-3 of the result.  Exact sums cost little where W's bytes bound the call (100 tokens of 8 experts of 1376
-    // 56 us, 50 without; 16 of 64 228, 223), but tiles half as much again (4096 tokens 1280 us, 830 without): there bf16 results,
+    // 56 us, 50 without; 16 of 64 228, 223), but tiles half as much again (4096 tokens 1240 us, 820 without): there bf16 results,
     // whose own rounding is 1.7e-3, go without (2.0e-3 together), and fp16 ones (3.3e-4) do not.
-    up.exact = a.dtype_c != TV_BFLOAT16;
+    up.exact = a.dtype_c != TV_BFLOAT16 || tk < kExactSlots;
     bool tiled = tk >= (int64_t)(pad_up ? kPadTileRows : pad_down ? kPadDownTileRows : up.exact ? kExactTileRows : kTileRows) * a.E && a.dtype_c != TV_FLOAT32 && a.I > 0;
     tiled = tiled && (!pad_up || fp8_pad_ok(up, FP8_GATE_UP)) && (!pad_down || fp8_pad_ok(down, FP8_DOWN));
     // Rows of up to `bm` make at most this many tiles.  A grid's threads are limited: calls beyond take the next kernel, the direct one

@@ -48,3 +48,17 @@ def test_fp32_results_are_exact(hip, t, h, i, e, k):
     assert (want.abs() < 2.0 ** 20).all() and (want * 16 == (want * 16).round()).all()
     off = (got.double().cpu() - want).abs()
     assert torch.equal(got.double().cpu(), want), f"{int((off > 0).sum())} of {off.numel()} off, by up to {float(off.max())}"
+
+
+@pytest.mark.parametrize("t,h,i,e,k", [(60, 1536, 512, 8, 4), (50, 512, 384, 8, 4), (250, 1536, 512, 8, 4)])
+def test_bf16_results_of_few_slots(hip, t, h, i, e, k):
+    """The error's norm against 64 bits, call by call: the rounding to bf16, at most 2^-8 / sqrt(3) of the result (half an ulp of
+    the smallest mantissa, evenly spread), and 2^-10 for the codes that exact sums still move and the second product.  Where the first
+    product's sums are cut, a few moved codes of large values make some of the calls several times worse."""
+    from tests.test_experts_gpu import make as layer
+    for seed in range(40):
+        args = layer(t, h, i, e, k, 1000 + seed)
+        want, _ = ref.experts(*args)
+        got = tv.experts_fp8(*args).double()
+        error = float((got - want).norm() / want.norm())
+        assert error <= 2.0 ** -8 / 3 ** 0.5 + 2.0 ** -10, (seed, error)
