@@ -310,12 +310,11 @@ int tv_hip_route(const tv_route_args* args, void* hip_stream);
  * [E, 2, ceil(I/128), ceil(H/128)] and [E, ceil(H/128), ceil(I/128)].  Slots with an id below 0 or not
  * below E have no expert and add nothing; a token without experts gets a row of zeros.
  * E <= TV_ROUTE_MAX_EXPERTS, k <= 64, T * k below 2^31 - 2^20.
- * Large calls (22 slots an expert and more, a 16-bit result) keep each slot's product, until the sum, as
- * fp16 with a power of two per 64 columns: a rounding to 11 bits before the one to dtype_c.  Block sums
- * of the first product are exact (see tv_gemm_fp8_args), but in such calls of 8192 slots and more with a BFLOAT16
- * result, whose two products both
- * use the 8-bit instructions; those of the second product are exact for a FLOAT32 result and the 8-bit instructions'
- * for 16-bit ones.
+ * Large calls with a 16-bit result (28 slots an expert and more; 22 in those of 8192 slots and a BFLOAT16 result; more where the weights'
+ * rows are not whole 16-byte chunks) keep each slot's product, until the sum, as fp16 with a power of two per 64 columns: a rounding
+ * to 11 bits before the one to dtype_c.  Block sums of the first product are exact (see tv_gemm_fp8_args), but in large
+ * calls of 8192 slots and more with a BFLOAT16 result the 8-bit instructions'; those of the second product are exact for a
+ * FLOAT32 result, the 8-bit instructions' for 16-bit ones.
  * Needs a workspace per stream, grown as tv_hip_gemm's is, of at most 5 I' + 4 H' + I' / 32 + 13 bytes a slot, I' = I
  * rounded up to 128, H' = H to 8, for the first 2^19 slots (more run in parts), and 16 E + 4096 more; TV_E_NOMEM, with nothing
  * launched, where it cannot be allocated.  Where there is room it also takes the partial sums of split products (16 MiB

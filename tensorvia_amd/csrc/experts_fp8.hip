@@ -162,7 +162,7 @@ struct ExpertScratch {
 };
 
 // Rows per expert (on average) from which the products take tiles through LDS, and tiles of 256 rows instead of 128.  us on
-// tiles / without, 64 experts of 1376, k = 8, bf16: 20 rows 272 / 257, 25 rows 277 / 297; fp16, whose block sums are exact: 24 rows 298 /
+// tiles / without, 64 experts of 1376, k = 8, tiles without exact sums: 20 rows 272 / 257, 25 rows 277 / 297; with exact sums: 24 rows 298 /
 // 262, 28 rows 286 / 304.  Where tiles need the weights in padded rows, copied on every call, from more: [T,4095], 64 experts of 1377, 64
 // rows 735 / 583, 96 rows 734 / 700, 128 rows 744 / 872; W2 alone, [T,2048], 16 experts of 1001, 75 rows 64 / 66.  64 rows: 333 in
 // tiles of 256, 338 of 128.

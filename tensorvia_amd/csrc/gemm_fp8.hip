@@ -13,7 +13,7 @@ namespace tvk {
 // Products of few rows: the weights stream from memory, so a workgroup takes 16 columns and 16 MT rows, and
 // its KW waves take every KW-th block of k; their sums meet in LDS.  Operands go straight from memory to
 // registers (no wave shares W with another, and A's few rows come from the caches).  Bound by W's bytes: [1,4096]x[11008,4096]
-// 8.7 us, 5.2 TB/s; up-projections of one token through 8 experts of 1376 (90 MB) 15.8 us, 5.7 TB/s.
+// 9.7 us, 4.7 TB/s; up-projections of one token through 8 experts of 1376 (90 MB) 16.6 us, 5.4 TB/s.
 //  FP8_DENSE    C [M, N] in dtype_c;
 //  FP8_GATE_UP  rows of one expert, gathered through row_token; both halves of W1, C = silu(gate) * up in fp32;
 //  FP8_SLOT_UP  the same without a plan: a tile is one slot;
@@ -158,8 +158,9 @@ __global__ __launch_bounds__(64 * KW) void gemm_fp8_direct_kernel(Fp8Gemm g) {
 // token's slots, one after the other, are a single long k, so the sum over slots is the accumulation (the routing
 // weight is part of the block's scale) and C is written once.  The inner rows [slots][ld] come in fp32: they are a
 // few kilobytes, which every workgroup quantises into LDS itself while its first weights are on their way.  With
-// plan, quantisation, product and sum as launches of their own one token of 64 experts of 1376, k = 8, took 46 us; it takes 31 (this
-// kernel 11.5 for 45 MB: its first loads and the quantisation are a third of it; four or six blocks in flight took 32.5 and 33.2).
+// plan, quantisation, product and sum as launches of their own one token of 64 experts of 1376, k = 8, took 46 us; it takes 31 to 33
+// (this kernel 12 for 45 MB: its first loads and the quantisation are a third of it; four or six blocks in flight took 32.5 and 33.2 where
+// three took 31).
 constexpr int kTokenWaves = 16, kTokenU = 3;
 
 template <typename TC, int ROWS>

@@ -6,8 +6,8 @@
 //  * A wave's tile is FM x FN blocks of 16 x 16.  Per k-tile each block is one matrix instruction into a fresh
 //    result and four multiply-adds that bring it, scaled, into the sum.  The result of a row of blocks is scaled while the
 //    next row's instructions run: 4 x 4 cycles of vector ALU per 32 cycles of matrix core.
-//  * bf16 [4096,4096]x[11008,4096]: 168 us, 2.2 PFLOP/s (3 rounds of 688 tiles on 256 CUs), the matrix cores busy for 52 % of the
-//    cycles and LDS for 25 %, at 2.0 GHz under the board's power limit: behind a k-tile's barrier its eight waves read their next
+//  * bf16 [4096,4096]x[11008,4096]: 173 to 180 us, 2.1 PFLOP/s (3 rounds of 688 tiles on 256 CUs; single launches between 167
+//    and 201), the matrix cores busy for 52 % of the cycles and LDS for 25 %, at 2.0 GHz under the board's power limit: behind a k-tile's barrier its eight waves read their next
 //    fragments all at once.  4096 tokens of 64 experts of 1376, k = 8: gate and up 420-440 us, down 310-320.
 //  * Scales of A's rows come through LDS beside the codes (one 4-byte direct load per row and k-tile); W's scale is
 //    one value per wave and k-tile, held 64 k-tiles at a time in one register across the lanes.
