@@ -6,8 +6,9 @@ consecutive elements of a row (activations: ``scale[m, k // 128]``) or of 128 x 
 ``scale[n // 128, k // 128]``).  The activation scales that these functions allocate are stored by column (a
 [blocks, rows] tensor, transposed): that is how the products read them fastest.  Any strides are accepted.
 
-Like ``gemm``, every function is asynchronous on ``stream`` (default torch's current one; what it allocates then
-belongs to that stream), takes the tensors to write as optional arguments, and raises RuntimeError for arguments that do not fit together or are not on a GPU.
+Like ``gemm``, every function is asynchronous on ``stream`` (default torch's current one; results that it allocates
+belong to that stream) and takes the tensors to write as optional arguments.  It raises RuntimeError for arguments that
+do not fit together or are not on a GPU.
 """
 from __future__ import annotations
 
@@ -95,9 +96,10 @@ def _codes_out(q, shape: tuple, device, stream) -> tuple:
 
 
 def _call(name: str, args: bytes, device, stream) -> None:
-    if device.type != "cuda":
+    index = device.index
+    if index is None:
         _fail(f"the tensors must be on a GPU, got {device}")
-    rc = _launch(name, args, device, stream)
+    rc = _launch(name, args, index, stream)
     if rc:
         check(rc)
 
